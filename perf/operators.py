@@ -276,8 +276,7 @@ def _adamw(s):
 
 def _adamw_out(s, norm):
     if s["case"]["bits"] == 8:
-        roots = s["opt"].read_state(moments=False)[1] if own else _values_r(s["r"], s["r_scale"])
-        out = {"p": s["p"], "m": s["m"], "m_scale": s["m_scale"], "r": roots, "r_scale": s["r_scale"]}
+        out = {"p": s["p"], "m": s["m"], "m_scale": s["m_scale"], "r": _values_r(s["r"], s["r_scale"]), "r_scale": s["r_scale"]}
     else:
         out = {"p": s["p"], "m": s["m"], "v": s["v"]}
     if s["case"]["master"]:
