@@ -1,5 +1,6 @@
 // version.cpp -- nerfhip_version(): release + the hash of the kernel sources this library was built from (Makefile: SRC_HASH,
-// sha256 over *.hip *.h *.inc of this directory).  A measurement file that records the string can be matched to a library.
+// sha256 over *.hip *.h *.inc of this directory without the operators': adamw*, ffn*, op_common.h).  A measurement file that
+// records the string can be matched to a library.
 #ifndef NERFHIP_SRC_HASH
 #define NERFHIP_SRC_HASH "unknown"
 #endif
