@@ -114,7 +114,8 @@ template <int ACT, bool SLOPE> __device__ __forceinline__ void activation(float 
     q = fmaf(q, s, 0.459120303f);
     q = fmaf(q, s, 1.15111494f);
     q = fmaf(q, s, 0.999999821f);
-    a = fmaf(0.5f, g + __builtin_fabsf(g), -s * __builtin_amdgcn_exp2f(-q));      // max(g, 0) that keeps a NaN
+    const float top = fmaf(0.5f, __builtin_fabsf(g), 0.5f * g);     // max(g, 0) that keeps a NaN; g + |g| would pass fp32's range
+    a = fmaf(-s, __builtin_amdgcn_exp2f(-q), top);
     da = 0.0f;
   } else if constexpr (ACT == NERFHIP_ACT_GELU) {
     const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678118654752f, __builtin_fabsf(g), 1.0f));
