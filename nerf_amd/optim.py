@@ -56,7 +56,7 @@ class _Handle:
 
     def set_stream(self, stream_ptr):
         """Run on this HIP stream from now on; None: on torch's current stream again.  New tensors (results, scratch memory) then belong
-        to that stream."""
+        to that stream.  It has to exist until a call has run on another one: what synchronises waits for the last call's stream."""
         import torch
         self._fixed = None if stream_ptr is None else torch.cuda.ExternalStream(stream_ptr, device=self._device)
         if stream_ptr is not None:
@@ -207,15 +207,21 @@ class AdamW(_Handle):
         self._chk(self._fn("read_state")(self._h, m.data_ptr() if moments else None, r.data_ptr() if roots else None), "read_state")
         return m, r
 
+    def _wait(self):
+        """For calls that synchronise: whatever stream the last call ran on has to be done with, not just the current one."""
+        self.synchronize()
+        self._follow()
+
     def get_step(self):
         """The number of updates so far (synchronises)."""
-        self._follow()
+        self._wait()
         t = C.c_int64()
         self._chk(self._fn("get_step")(self._h, C.byref(t)), "get_step")
         return t.value
 
     def set_step(self, step):
-        self._follow()
+        """Makes this the number of updates so far (synchronises)."""
+        self._wait()
         self._chk(self._fn("set_step")(self._h, int(step)), "set_step")
 
     def state_dict(self):
