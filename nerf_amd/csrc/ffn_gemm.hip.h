@@ -154,13 +154,18 @@ __device__ __forceinline__ float activation_value(int act, float g) {
   return a;
 }
 
-// three bf16 pieces of a float: truncated, so that the remainders are exact and no finite value becomes infinite
+// Three bf16 pieces of a float, each what is left rounded to nearest: after the first at most 2^-8, after the second 2^-17 of the power of two
+// below |x|, and the third is exact.  The first is kept finite for finite x (what is left of 2^128 - 2^104 has 16 bits); an infinity leaves an
+// infinity and then a NaN, a NaN itself.  Cut off instead of rounded, all pieces had x's sign, and the products left out up to 2^-21 of the
+// whole, always towards zero.
 __device__ __forceinline__ void split3(float x, uint16_t (&p)[3]) {
+  constexpr float kTop = 3.38953139e38f;      // the largest bf16
+  float y = __builtin_amdgcn_fmed3f(x, -kTop, kTop);
 #pragma unroll
   for (int i = 0; i < 3; ++i) {
-    const uint32_t b = __builtin_bit_cast(uint32_t, x) & 0xffff0000u;
-    p[i] = (uint16_t)(b >> 16);
-    x -= __builtin_bit_cast(float, b);
+    const __bf16 q = (__bf16)y;
+    p[i] = __builtin_bit_cast(uint16_t, q);
+    y = x -= (float)q;
   }
 }
 
