@@ -69,7 +69,7 @@ def _close(got, want, rel, name):
 
 
 # 64 x 128, 128 x 128 and 256 x 256 tiles; the gate, dh and the weight gradients whole and in parts; sizes that end inside a tile
-SIZES = [(65, 64), (100, 1024), (300, 264), (1000, 72), (2048, 2048), (16384, 512), (9000, 257)]
+SIZES = [(65, 64), (100, 1024), (300, 264), (1000, 72), (2048, 2048), (16384, 512), (9000, 257), (524, 549), (34000, 256)]
 
 
 @pytest.mark.parametrize("full", ["first", "down"])
