@@ -285,8 +285,8 @@ typedef struct nerfhip_ffn_config {
   int32_t dtype;       /* of every tensor: NERFHIP_F32 | NERFHIP_BF16 | NERFHIP_F16.  Sums are held in fp32; h, dg and du are
                         * rounded to 16 bits for the next product when the tensors are (h of up to 16 rows is not; in F16
                         * what passes 65504 becomes infinite).  F32 products of more than 64 rows, and of the backward pass, are formed from three bf16 pieces of each
-                        * operand (24 bits; what lies below 2^-133 is dropped): finite values give fp32 results, a product with
-                        * an infinite or NaN operand gives NaN. */
+                        * operand (24 bits; what lies below 2^-133 is dropped): finite values give fp32 results (a product is off by 2^-24
+                        * of itself at most, beside its rounding), a product with an infinite or NaN operand gives NaN. */
   int32_t activation;  /* NERFHIP_ACT_* */
   int32_t bias;        /* 0: no biases; 1: b_gate, b_up [d_ff], b_down [d_model] */
   int32_t device;
@@ -307,7 +307,8 @@ void nerfhip_ffn_destroy(nerfhip_ffn_t* h);
 const char* nerfhip_ffn_last_error(const nerfhip_ffn_t* h);   /* NULL: the last nerfhip_ffn_create error of this thread */
 int nerfhip_ffn_set_stream(nerfhip_ffn_t* h, void* hip_stream);
 int nerfhip_ffn_synchronize(nerfhip_ffn_t* h);
-/* Bytes of scratch memory that a call with this many rows needs (256-byte aligned).  Its contents mean nothing between
+/* Bytes of scratch memory that a call with this many rows needs (256-byte aligned).  They go by the rows alone, so that they include room for
+ * copies of x, dy and the weights, which 16-bit tensors need where a row does not start or end at 16 bytes.  Its contents mean nothing between
  * calls; calls that run at the same time -- two streams, two graphs -- need scratch of their own.  -1: bad argument. */
 int64_t nerfhip_ffn_workspace_bytes(const nerfhip_ffn_t* h, int64_t rows, int32_t backward);
 /* rows: 0 .. 2^31 - 1024.  ldx, ldy: elements between rows, as the weights' ld at most 2097152.  Otherwise strides, sizes and addresses may be
@@ -373,7 +374,8 @@ int nerfhip_adamw_grad_norm(nerfhip_adamw_t* h, double max_norm, double loss_sca
  * starting at a multiple of 256 values (what lies between is set to 0).  Device pointers, either may be NULL; they may not overlap
  * the tensors. */
 int nerfhip_adamw_read_state(nerfhip_adamw_t* h, float* m, float* root);
-/* The update count lives on the device (a captured step counts its replays); both calls synchronise with the stream. */
+/* The update count lives on the device (a captured step counts its replays); both calls synchronise with the handle's stream: steps
+ * on a stream that set_stream named before have to be waited for first (synchronize, before set_stream). */
 int nerfhip_adamw_get_step(nerfhip_adamw_t* h, int64_t* step);
 int nerfhip_adamw_set_step(nerfhip_adamw_t* h, int64_t step);
 

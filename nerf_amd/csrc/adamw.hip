@@ -5,7 +5,8 @@
 // Bound by memory: per value p in and out, g in, m and v in and out -- 28 bytes all in fp32, 10 with 16-bit p and g and
 // 8-bit states.  The tensors are cut at create time into chunks whose records (addresses, length, decay) lie in device
 // memory, so a workgroup reaches its data by ONE dependent load; a fixed grid walks over the records.  Measured: 201 M bf16 values with
-// fp32 copies and states 1115 us (5.0 TB/s), with 8-bit states and no copies 440 - 515 us (3.9 - 4.6 TB/s), their norm 70 us (5.7 TB/s); a million
+// fp32 copies and states 1116 us (5.0 TB/s), with 8-bit states and no copies 437 us in a kernel trace, 450 - 540 from run to run of calls in a row (3.8 -
+// 4.6 TB/s), their norm 70 us where nothing else runs (5.7 TB/s: of 403 MB the chip's last cache keeps a part), 92 - 117 in front of a step; a million
 // values of 48 tensors in fp32 6.2 us, which is the chain record -> data -> store.  1280 or 4096 workgroups instead of at most 2048, and
 // chunks of 16 passes instead of 4, take the same; chunks of one pass for 201 M values 1220 us.
 //

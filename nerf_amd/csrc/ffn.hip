@@ -41,7 +41,7 @@ template <class V> __device__ __forceinline__ V load_any(const void* p) {
 // ---- few rows: the weights are read once, straight into registers ------------------------------------------------------
 // One workgroup: 16 output columns (GATE: of both weights), its NW waves take every NW-th piece of kUnroll x 64 bytes of k; lane (c, g)
 // reads 16 bytes of weight row c, k chunk g, which is what the matrix instruction wants.  Bound by the weights' bytes: 8 rows of
-// 4096 -> 2 x 16384 -> 4096 in bf16, 403 MB, take 50 + 36 us.
+// 4096 -> 2 x 16384 -> 4096 in bf16, 403 MB, take 86 us, 50 and 36.
 // Where 16 columns each would leave CUs without a workgroup and rows are few, P parts of k take the place of rows and columns: row c of both
 // operands is row or column c % (16 / P) of part c / (16 / P), and of the products the P squares on the diagonal count.  One row of
 // 4096 -> 1024: 4.5 us with four parts, 8.1 with one; past one workgroup to a CU they lose (2 rows of 4096 -> 4096: 8.5 us with one, 9.0

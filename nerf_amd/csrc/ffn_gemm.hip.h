@@ -5,9 +5,9 @@
 // An operand lies in memory either with its k values consecutive ([m][k]) or with its m values consecutive ([k][m]); both
 // occur: forward products read rows of x and W, dx reads W by columns, the weight gradients read both operands by columns.
 // A segment is one pair of operands; the sum over segments stays in the accumulators: dx = dg Wg + du Wu is two.  An fp32 operand is three
-// planes of bf16 pieces of 8 bits (x = x0 + x1 + x2 exactly), and its product the sum of x2 w0, x0 w2, x1 w1, x1 w0, x0 w1, x0 w0, which
-// leaves out what is below 2^-24 of the whole.  One product after the other, the smallest first, rounds least: sums over 65536 rows of what
-// comes out were 3.5e-7 off, and 1.6e-6 with all six for the same 64 k, where every one rounds at the full sum.  The weight gradients take
+// planes of bf16 pieces of 8 bits (x = x0 + x1 + x2 exactly, each rounded to nearest), and its product the sum of x2 w0, x0 w2, x1 w1, x1 w0, x0 w1,
+// x0 w0, which leaves out at most 2^-24 of the whole, of either sign.  One product after the other, the smallest first, rounds least: sums over
+// 65536 rows of what comes out are 3.3e-7 off, and 1.3e-6 with all six for the same 64 k, where every one rounds at the full sum.  The weight gradients take
 // the second order all the same: their long k comes from memory, and in the first order each plane two and three times (914 TFLOP/s of the
 // six products against 1330 of a single one; 1200 then).  Both stay below what an fp32 sum over so many rows loses.
 //
@@ -21,9 +21,10 @@
 //     eight rows that a half wave reads at once then lie in eight different bank groups.
 // A direct load writes LDS linearly in lane order, so the permutations are applied to the lanes' global addresses.
 //
-// Bound by the matrix unit (and the clock that its power leaves) where sums are long: 8192 rows of 2048 -> 8192 in bf16, dx 1440 - 1470 TFLOP/s,
-// weight gradients 1340 - 1400, dh, whose 268 MB of fp32 results are stored too, 1170.  Short sums leave the epilogue: the gate of 262144
-// rows of 256 -> 2 x 1024 in 390 - 430 us with gelu and biases is 196 of products, 0.54 GB of h and 64 activations a lane for four steps.
+// Bound by the matrix unit (and the clock that its power leaves) where sums are long: 8192 rows of 2048 -> 8192 in bf16, dx 1430 TFLOP/s,
+// weight gradients 1340, dh, whose 268 MB of fp32 results are stored too, 1170 (kernel trace, calls in a row, on a card where the library's
+// product of 8192^3 reaches 1370; 5 % more on the best one).  Short sums leave the epilogue: the gate of 262144
+// rows of 256 -> 2 x 1024 in 407 us with gelu and biases is 196 of products, 0.54 GB of h and 64 activations a lane for four steps.
 //
 // The product is formed as v_mfma_f32_16x16x32 with the B rows as its first operand: a lane then holds four consecutive n of
 // one row m, which the epilogues store as one piece.
