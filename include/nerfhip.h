@@ -375,7 +375,7 @@ int nerfhip_adamw_grad_norm(nerfhip_adamw_t* h, double max_norm, double loss_sca
  * the tensors. */
 int nerfhip_adamw_read_state(nerfhip_adamw_t* h, float* m, float* root);
 /* The update count lives on the device (a captured step counts its replays); both calls synchronise with the handle's stream: steps
- * on a stream that set_stream named before have to be waited for first (synchronize, before set_stream). */
+ * on a stream that set_stream named before, and graphs replayed on other streams, have to be waited for first. */
 int nerfhip_adamw_get_step(nerfhip_adamw_t* h, int64_t* step);
 int nerfhip_adamw_set_step(nerfhip_adamw_t* h, int64_t step);
 

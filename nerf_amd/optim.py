@@ -213,14 +213,15 @@ class AdamW(_Handle):
         self._follow()
 
     def get_step(self):
-        """The number of updates so far (synchronises)."""
+        """The number of updates so far.  Waits for the last call's stream and the current one; a graph that is replayed on a third has to
+        be waited for before."""
         self._wait()
         t = C.c_int64()
         self._chk(self._fn("get_step")(self._h, C.byref(t)), "get_step")
         return t.value
 
     def set_step(self, step):
-        """Makes this the number of updates so far (synchronises)."""
+        """Makes this the number of updates so far; waits as get_step does."""
         self._wait()
         self._chk(self._fn("set_step")(self._h, int(step)), "set_step")
 
